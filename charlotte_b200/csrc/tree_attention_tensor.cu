@@ -685,12 +685,17 @@ __device__ __noinline__ void bring(Info& info, char* smem) {
             char* const ring = smem + F::kRingAt + kind * (F::kRing * kTile * D);
             const uint32_t own = key0 * D + ((piece0 ^ ((D == 128 ? sub : sub / 2u) & kSwap)) << 4);
             static_assert(kSub == 1, "a thread's piece is the same of all its rows");
+            // rfull has one arrival a tile, the first warp's, which is made only
+            // once every warp is done with the slot's tile before, however this
+            // one comes: so the barrier is never two phases ahead of a warp that
+            // is still at that tile (it would take the parity of the later phase
+            // for one not yet done), and no copy lands on codes still unread.
             auto fetch = [&](uint32_t t) {
                 if (t < n) {
                     const uint32_t it = done + t, r = it % F::kRing;
+                    if (w == 0 && lane == 0) wait(&info.rempty[kind][r], (it / F::kRing & 1u) ^ 1u, info);
                     if (whole(t)) {
                         if (w == 0 && lane == 0) {
-                            wait(&info.rempty[kind][r], (it / F::kRing & 1u) ^ 1u, info);
                             mbar_arrive_expect_tx(&info.rfull[kind][r], kTile * D);
                             copy_tile(ring + r * kTile * D, map, 0, on.h, slot_at(at0 + t * kTile), on.s, &info.rfull[kind][r]);
                         }
