@@ -218,13 +218,13 @@ __global__ void __launch_bounds__(64) verify_kernel(const VerifyArgs args) {
             const uint32_t t = __shfl_sync(kAll, i < 32u ? id[0] : id[1], i & 31u);
             const float draw = __shfl_sync(kAll, i < 32u ? u[0] : u[1], i & 31u);
             const float p = of_token(r, t);
-            float q_raw = 1.0f, divisor = 1.0f;
+            float q_of = 1.0f;
             if (have) {
-                divisor = mass > 0.0f ? mass : 1.0f;
-                q_raw = of_token(q, t);
-                if (!(q_raw > 0.0f)) continue;
+                q_of = of_token(q, t);
+                if (!(q_of > 0.0f)) continue;
+                q_of /= mass;
             }
-            if (draw * (q_raw / divisor) < p) {
+            if (draw * q_of < p) {
                 next = i;
                 break;
             }
@@ -242,25 +242,28 @@ __global__ void __launch_bounds__(64) verify_kernel(const VerifyArgs args) {
                         }
                     }
                 }
-                const float scale = 1.0f / divisor;
-                rest[0] = fmaxf(r.p[0] - on_target[0] * scale, 0.0f);
-                rest[1] = fmaxf(r.p[1] - on_target[1] * scale, 0.0f);
+                rest[0] = fmaxf(r.p[0] - on_target[0] / mass, 0.0f);   // a subnormal mass has no finite inverse
+                rest[1] = fmaxf(r.p[1] - on_target[1] / mass, 0.0f);
             } else {
                 rest[0] = r.token[0] == t ? 0.0f : r.p[0];
                 rest[1] = r.token[1] == t ? 0.0f : r.p[1];
+            }
+            if (have) {
+                // What is left of q, summed and not one less what is gone: a draft
+                // sure of its first token leaves its siblings 1e-8 and less, which
+                // that difference rounds away. Nothing left: every later sibling's
+                // probability is 0, and it is refused.
+                forget(q, t);
+                mass = warp_sum(q.p[0] + q.p[1]);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (r.token[c] == t) on_target[c] = 0.0f;
             }
             const float total = warp_sum(rest[0] + rest[1]);
             if (total > 0.0f) {
                 const float scale = 1.0f / total;
                 r.p[0] = rest[0] * scale;
                 r.p[1] = rest[1] * scale;
-            }
-            if (have) {
-                mass -= q_raw;
-                forget(q, t);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    if (r.token[c] == t) on_target[c] = 0.0f;
             }
         }
         if (next == kAbsent) break;
