@@ -86,7 +86,7 @@ __device__ bool distribution(const uint32_t* pairs, const cb_sampling& s, float 
         const float a = kept[0] ? exp_nonpositive(gap[0]) : 0.0f, b = kept[1] ? exp_nonpositive(gap[1]) : 0.0f;
         const float before = sum_before(a, b, lane);
         const float scale = 1.0f / __shfl_sync(kAll, before + a + b, 31);
-        kept[0] = kept[0] && before * scale < s.top_p;
+        kept[0] = kept[0] && (lane == 0 || before * scale < s.top_p);   // the first stays, whatever top_p is
         kept[1] = kept[1] && (before + a) * scale < s.top_p;
     }
     if (s.min_p != 0.0f) {
