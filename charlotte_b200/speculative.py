@@ -138,6 +138,12 @@ class SpeculativeDecoder:
             self._norm(self.output_norm, post, True)
             self._product([self.head], self.normed, [self.logits])
 
+    def _within_context(self, lengths, rows) -> None:
+        """rows: positions past its length that each sequence needs."""
+        for s, (length, n) in enumerate(zip(lengths, rows)):
+            if n and length + n > self.arch.context:
+                raise ValueError(f"sequence {s}: positions past the context of {self.arch.context} ({length} + {n})")
+
     def _set(self, trees) -> None:
         """trees: for each sequence its rows' (tokens, ancestor masks); no rows: it takes no part."""
         ids = np.zeros((self.sequences, self.nodes), np.uint32)
@@ -152,7 +158,9 @@ class SpeculativeDecoder:
     # ---- steps ------------------------------------------------------------------------
 
     def prefill(self, prompts) -> None:
-        """Writes each sequence's prompt but its last token, which the first step takes as its row 0."""
+        """Writes each sequence's prompt but its last token, which the first step takes as its row 0. A prompt that does
+        not fit its sequence's context is a ValueError, and nothing runs."""
+        self._within_context(self.lengths.tolist(), [len(p) - 1 for p in prompts])
         done = [0] * self.sequences
         while any(d < len(p) - 1 for d, p in zip(done, prompts)):
             trees = []
@@ -169,15 +177,10 @@ class SpeculativeDecoder:
         after its parent. `sampling`, `draft_sampling`: dicts of temperature, top_k, top_p, min_p (default: greedy);
         `uniforms` [sequences, nodes] (not for greedy drafts of a greedy target); `draft`: the drafting model's
         candidates [sequences, nodes, 64, 2] (int32, cuda), None where each drafted token was certain. Returns each
-        sequence's new tokens, the last of them the next tree's row 0."""
-        masks = []
-        for tokens, parents in trees:
-            m = []
-            for i, parent in enumerate(parents):
-                if not (parent == -1 and i == 0 or 0 <= parent < i):
-                    raise ValueError(f"row {i} comes before its parent {parent}")
-                m.append((m[parent] if parent >= 0 else 0) | 1 << i)
-            masks.append((tokens, m))
+        sequence's new tokens, the last of them the next tree's row 0. A tree with a row past the context is a ValueError,
+        and nothing runs."""
+        masks = [(tokens, ancestors(parents)) for tokens, parents in trees]
+        self._within_context(self.lengths.tolist(), [max((x.bit_count() for x in m), default=0) for _, m in masks])
         self._set(masks)
         self._forward(logits=True)
         a, rows = self.arch, self.ids.shape[0]
@@ -198,8 +201,10 @@ class SpeculativeDecoder:
 
     def generate(self, prompts, count: int, drafter=None, sampling=None, seed: int = 0):
         """`count` new tokens of each prompt (at least; lists of ints), drafted by `drafter(tokens so far, rows)` ->
-        (tokens, parents) of the rows after row 0, parents counted with it. Returns (the new tokens, steps taken)."""
+        (tokens, parents) of the rows after row 0, parents counted with it; rows past the context are left out. Returns
+        (the new tokens, steps taken). A ValueError where a prompt and its tokens but the last do not fit the context."""
         drafter = drafter or lookup
+        self._within_context([len(p) for p in prompts], [max(count - 1, 0)] * len(prompts))
         self.lengths.zero_()
         self.prefill(prompts)
         rng = np.random.default_rng(seed)
@@ -211,12 +216,31 @@ class SpeculativeDecoder:
                     trees.append(([], []))
                     continue
                 tokens, parents = drafter(t, self.nodes)
-                trees.append(([t[-1], *tokens], [-1, *parents]))
+                trees.append(less_deep([t[-1], *tokens], [-1, *parents], self.arch.context - len(t) + 1))
             u = self.torch.from_numpy(rng.random((self.sequences, self.nodes), np.float32)) if sampling else None
             for t, new in zip(told, self.step(trees, sampling, u)):
                 t.extend(new)
             steps += 1
         return [t[len(p):] for t, p in zip(told, prompts)], steps
+
+
+def ancestors(parents) -> list[int]:
+    """The rows' ancestor masks: bit j of row i's is set when row j is an ancestor of it or i itself."""
+    masks = []
+    for i, parent in enumerate(parents):
+        if not (parent == -1 and i == 0 or 0 <= parent < i):
+            raise ValueError(f"row {i} comes before its parent {parent}")
+        masks.append((masks[parent] if parent >= 0 else 0) | 1 << i)
+    return masks
+
+
+def less_deep(tokens, parents, depth: int):
+    """The tree's rows of a depth below `depth` (row 0's is 0): a row's descendants go with it."""
+    place = {-1: -1}
+    for i, m in enumerate(ancestors(parents)):
+        if m.bit_count() <= depth:
+            place[i] = len(place) - 1
+    return [tokens[i] for i in place if i >= 0], [place[parents[i]] for i in place if i >= 0]
 
 
 def lookup(told, rows: int, most: int = 3):
