@@ -20,6 +20,7 @@ from . import model as M
 from . import synth
 
 MOST_NODES = 64
+DRAW = dict(temperature=0.0, top_k=64, top_p=1.0, min_p=0.0)   # a draw's settings where none are given
 
 
 class SpeculativeDecoder:
@@ -174,11 +175,14 @@ class SpeculativeDecoder:
 
     def step(self, trees, sampling=None, uniforms=None, draft=None, draft_sampling=None):
         """One step of each sequence's tree: (tokens, parents), row 0 the sequence's last token (parent -1) and a row
-        after its parent. `sampling`, `draft_sampling`: dicts of temperature, top_k, top_p, min_p (default: greedy);
-        `uniforms` [sequences, nodes] (not for greedy drafts of a greedy target); `draft`: the drafting model's
+        after its parent. `sampling`, `draft_sampling`: dicts of temperature, top_k, top_p, min_p, what they leave out as
+        in DRAW (greedy); `uniforms` [sequences, nodes], which a target with a temperature needs; `draft`: the drafting model's
         candidates [sequences, nodes, 64, 2] (int32, cuda), None where each drafted token was certain. Returns each
         sequence's new tokens, the last of them the next tree's row 0. A tree with a row past the context is a ValueError,
         and nothing runs."""
+        target = DRAW | (sampling or {})
+        if target["temperature"] > 0 and uniforms is None:
+            raise ValueError("a target with a temperature draws by uniform numbers, and none are given")
         masks = [(tokens, ancestors(parents)) for tokens, parents in trees]
         self._within_context(self.lengths.tolist(), [max((x.bit_count() for x in m), default=0) for _, m in masks])
         self._set(masks)
@@ -188,10 +192,9 @@ class SpeculativeDecoder:
             candidates=self.candidates, rows=rows, logits_stride=a.vocab, candidates_only=1)
         if uniforms is not None:
             self.uniforms.copy_(uniforms)
-        greedy = dict(temperature=0.0, top_k=1, top_p=1.0, min_p=0.0)
         plan("verify", candidates=self.candidates, draft_candidates=draft, ids=self.ids, uniforms=self.uniforms,
              nodes=self.live, ancestors=self.masks, path=self.path, kept=self.kept, sampled=self.sampled,
-             sequences=self.sequences, tokens=self.nodes, target=sampling or greedy, draft=draft_sampling or greedy)()
+             sequences=self.sequences, tokens=self.nodes, target=target, draft=DRAW | (draft_sampling or {}))()
         for keep in self.keeps:
             keep()
         self.lengths.copy_(self.new_lengths)
