@@ -15,7 +15,7 @@ import math
 
 import numpy as np
 
-from . import CACHE_F16, CACHE_Q8, GATED, QKV, WRITE, lib, matmul, plan, rope_turns, run  # noqa: F401
+from . import CACHE_Q8, GATED, QKV, CharlotteError, check, lib, matmul, plan, rope_turns, run
 from . import model as M
 from . import synth
 
@@ -156,13 +156,18 @@ class SpeculativeDecoder:
         put(self.masks, masks.view(np.int64))
         put(self.live, np.array([len(t) for t, _ in trees], np.int32))
 
+    def _check_waits(self) -> None:
+        """A CharlotteError where a bounded wait of a kernel ran out, and its results are no step's."""
+        self.torch.cuda.current_stream().synchronize()
+        check(lib().cb_fault_check(None))
+
     # ---- steps ------------------------------------------------------------------------
 
     def prefill(self, prompts) -> None:
         """Writes each sequence's prompt but its last token, which the first step takes as its row 0. A prompt that does
         not fit its sequence's context is a ValueError, and nothing runs."""
         self._within_context(self.lengths.tolist(), [len(p) - 1 for p in prompts])
-        done = [0] * self.sequences
+        done, start = [0] * self.sequences, self.lengths.clone()
         while any(d < len(p) - 1 for d, p in zip(done, prompts)):
             trees = []
             for s, p in enumerate(prompts):
@@ -172,6 +177,11 @@ class SpeculativeDecoder:
             self._set(trees)
             self._forward(logits=False)
             self.lengths += self.live
+        try:
+            self._check_waits()
+        except CharlotteError:
+            self.lengths.copy_(start)
+            raise
 
     def step(self, trees, sampling=None, uniforms=None, draft=None, draft_sampling=None):
         """One step of each sequence's tree: (tokens, parents), row 0 the sequence's last token (parent -1) and a row
@@ -179,7 +189,7 @@ class SpeculativeDecoder:
         in DRAW (greedy); `uniforms` [sequences, nodes], which a target with a temperature needs; `draft`: the drafting model's
         candidates [sequences, nodes, 64, 2] (int32, cuda), None where each drafted token was certain. Returns each
         sequence's new tokens, the last of them the next tree's row 0. A tree with a row past the context is a ValueError,
-        and nothing runs."""
+        and nothing runs; a kernel whose wait ran out is a CharlotteError, and the step can be taken again."""
         target = DRAW | (sampling or {})
         if target["temperature"] > 0 and uniforms is None:
             raise ValueError("a target with a temperature draws by uniform numbers, and none are given")
@@ -197,8 +207,9 @@ class SpeculativeDecoder:
              sequences=self.sequences, tokens=self.nodes, target=target, draft=DRAW | (draft_sampling or {}))()
         for keep in self.keeps:
             keep()
-        self.lengths.copy_(self.new_lengths)
         path, kept, sampled = (x.cpu().numpy() for x in (self.path, self.kept, self.sampled))
+        self._check_waits()   # before the lengths, so that a failed step's rows are no entries
+        self.lengths.copy_(self.new_lengths)
         return [[int(trees[s][0][i]) for i in path[s, 1:kept[s]]] + [int(sampled[s, 0])] if kept[s] else []
                 for s in range(self.sequences)]
 
