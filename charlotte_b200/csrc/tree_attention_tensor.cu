@@ -42,9 +42,9 @@
 // along d (K-major) they are K·Q^T's A, read along the keys (MN-major) P·V's
 // B. P is written key by key, a lane its key's weights: MN-major A.
 //
-// Every wait is bounded: one that runs out sets the fault word and `abort`,
-// after which every wait returns at once and the kernel runs to its end with
-// whatever it has (the host reports the step as failed).
+// Every wait is bounded: one that runs out sets the fault word (which
+// cb_fault_check reports) and `abort`, after which the other waits run out too
+// and the kernel runs to its end with whatever it has.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -151,7 +151,7 @@ struct Info {
     uint32_t unset[2];         // a half's live rows that have seen no key yet
     float least_unit[2];       // of the rows that have
     uint32_t latest, context;  // tiles from one to before the other are seen whole by every row
-    uint32_t last, abort, tmem;
+    uint32_t last, abort, polls, tmem;
     uint32_t first_cta, last_cta;   // of a divided pair
     bool begins;                    // whether its tiles begin inside the first one's share
     float2 scales[kScaleTiles][kTile];   // an 8-bit tile's key and value scales
@@ -233,17 +233,28 @@ __device__ __forceinline__ bool half_any(uint32_t half, bool p) {
     return r != 0;
 }
 
-// A wait never changes what a thread does next, so barriers stay matched
-// whatever runs out.
+// A wait never changes where a thread goes next, so that the barriers of whole
+// warps stay matched whatever runs out. It is looked at (`sound`) before the
+// arrivals that stand on it: those on a barrier that counts a copy's bytes,
+// which must not come before its phase is done, and the commits that let the
+// loaders on.
+__device__ __forceinline__ void ran_out(Info& info) {
+    *reinterpret_cast<volatile uint32_t*>(&info.abort) = 1u;
+    if (info.fault) atomicOr(info.fault, kFaultTimeout);
+}
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Info& info) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return;
-        if (i % 16u == 15u && *reinterpret_cast<volatile uint32_t*>(&info.abort)) return;
+        if (i % 16u == 15u) {
+            if (*reinterpret_cast<volatile uint32_t*>(&info.abort)) return;
+            if (i >= info.polls) break;
+        }
     }
-    *reinterpret_cast<volatile uint32_t*>(&info.abort) = 1u;
-    if (info.fault) atomicOr(info.fault, kFaultTimeout);
+    ran_out(info);
 }
+// Whether every wait of the CTA was met so far, this thread's own among them.
+__device__ __forceinline__ bool sound(const Info& info) { return *reinterpret_cast<const volatile uint32_t*>(&info.abort) == 0u; }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -428,6 +439,7 @@ __device__ __forceinline__ void issue_scores(Info& info, uint32_t base, uint32_t
     wait(&info.sempty[sb], (it >> 1 & 1u) ^ 1u, info);
     tc_fence_after();
     if (lane == 0) {
+        const bool go = sound(info);
         asm volatile("" : "+r"(base));   // descriptors are made here, not kept in registers through the softmax
         const uint64_t da = umma_desc_sw128(base + F::kKeysAt + st * F::kOperand), db = umma_desc_sw128(base);
 #pragma unroll
@@ -437,8 +449,10 @@ __device__ __forceinline__ void issue_scores(Info& info, uint32_t base, uint32_t
                 umma_f16(tmem + sb * F::RT, da + k / 4u * (kPiece >> 4) + k % 4u * 2u,
                          db + (1u - term) * (F::RT * 128u >> 4) + k / 4u * (F::N * 128u >> 4) + k % 4u * 2u,
                          umma_idesc_f16(kTile, F::RT), term + k > 0);
-        umma_commit(&info.kempty[st]);
-        umma_commit(&info.sfull[sb]);
+        if (go) {
+            umma_commit(&info.kempty[st]);
+            umma_commit(&info.sfull[sb]);
+        }
     }
     __syncwarp();
 }
@@ -450,14 +464,17 @@ __device__ __forceinline__ void issue_sums(Info& info, uint32_t base, uint32_t t
     wait(&info.pfull[pb], it / F::kWeights & 1u, info);
     tc_fence_after();
     if (lane == 0) {
+        const bool go = sound(info);
         asm volatile("" : "+r"(base));
         const uint64_t da = desc_mn(base + F::kPAt + pb * F::kP), db = desc_mn(base + F::kValuesAt + st * F::kOperand);
 #pragma unroll
         for (uint32_t k = 0; k < kTile / 16u; ++k)
             umma_f16(tmem + F::kSumsAt, da + k * (2048u >> 4), db + k * (2048u >> 4), umma_idesc_f16(128, F::D) | kBothMn,
                      (it - first) % kFold != 0 || k > 0);
-        umma_commit(&info.vempty[st]);
-        umma_commit(&info.pempty[pb]);
+        if (go) {
+            umma_commit(&info.vempty[st]);
+            umma_commit(&info.pempty[pb]);
+        }
     }
     __syncwarp();
 }
@@ -574,6 +591,7 @@ __device__ __noinline__ void soften(Info& info, char* smem, uint32_t tmem) {
 template <class F>
 __device__ __noinline__ void multiply(Info& info, char* smem, uint32_t tmem) {
     const uint32_t lane = threadIdx.x & 31u, base = smem_addr(smem), n = info.on.n, done = info.on.done;
+    if (info.polls == 0u) ran_out(info);   // a wait given no poll at all
     for (uint32_t t = 0; t < n; ++t) {
         issue_scores<F>(info, base, tmem, done + t, lane);
         if (t > 1u) issue_sums<F>(info, base, tmem, done + t - 2u, done, lane);
@@ -650,7 +668,7 @@ __device__ __noinline__ void bring(Info& info, char* smem) {
     auto landed = [&](uint32_t st) {
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[st]);
+        if (lane == 0 && (F::Q8 || sound(info))) mbar_arrive(&full[st]);   // codes' copies count on barriers of their own
     };
     if constexpr (F::Q8) {
         // A tile's codes as f16 values, in the operand's swizzle.
@@ -695,7 +713,7 @@ __device__ __noinline__ void bring(Info& info, char* smem) {
                     const uint32_t it = done + t, r = it % F::kRing;
                     if (w == 0 && lane == 0) wait(&info.rempty[kind][r], (it / F::kRing & 1u) ^ 1u, info);
                     if (whole(t)) {
-                        if (w == 0 && lane == 0) {
+                        if (w == 0 && lane == 0 && sound(info)) {
                             mbar_arrive_expect_tx(&info.rfull[kind][r], kTile * D);
                             copy_tile(ring + r * kTile * D, map, 0, on.h, slot_at(at0 + t * kTile), on.s, &info.rfull[kind][r]);
                         }
@@ -704,7 +722,7 @@ __device__ __noinline__ void bring(Info& info, char* smem) {
                         each(t, 0, kEach, [&](uint32_t i, const char* src, bool there) {
                             copy16(ring + r * kTile * D + own + i * (kStep * D), src, there);
                         });
-                        if (w == 0 && lane == 0) mbar_arrive(&info.rfull[kind][r]);
+                        if (w == 0 && lane == 0 && sound(info)) mbar_arrive(&info.rfull[kind][r]);
                     }
                     if (!value) copy_scales(t);
                 }
@@ -761,12 +779,13 @@ __device__ __noinline__ void bring(Info& info, char* smem) {
             wait(&empty[st], (it / F::kStages & 1u) ^ 1u, info);
             char* to = operand + st * F::kOperand;
             if (whole(t)) {   // straight into the operand's layout
-                if (w == 0 && lane == 0) {
+                const bool arrives = lane == 0 && sound(info);
+                if (w == 0 && arrives) {
                     mbar_arrive_expect_tx(&full[st], F::kOperand);
 #pragma unroll
                     for (uint32_t d = 0; d < D / 64u; ++d)
                         copy_tile(to + d * kPiece, map, d * 64u, on.h, slot_at(at0 + t * kTile), on.s, &full[st]);
-                } else if (lane == 0) {
+                } else if (arrives) {
                     mbar_arrive(&full[st]);
                 }
                 __syncwarp();
@@ -878,6 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_tensor_kernel(cons
             }
         }
         info.abort = 0;
+        info.polls = min(spin_limit_of(args.fault), kPolls);
         info.fault = args.fault;
         fence_barrier_init();
     }

@@ -67,12 +67,13 @@ CB_API int cb_fault_check(unsigned int* faults);
 
 /* A test hook for failure detection (no counterpart in the reference): on
  * the current device, the first wait of each kernel on a bulk copy (the
- * decode products and decode attention) gives up after `polls` polls (0:
- * at once, without polling) instead of the full bound, so a test can make a
- * wait run out — the kernel records the timeout in the fault word, drains
- * its copies (with the full bound) and returns — without any fault. A
- * negative value restores the full bound. Read by the kernels when they run
- * (captured graphs included); set it only between steps. Synchronous. */
+ * decode products and decode attention; in tree attention's tcgen05 form
+ * every wait, in steps of 16 polls) gives up after `polls` polls (0: at once)
+ * instead of the full bound, so a test can make a wait run out — the kernel
+ * records the timeout in the fault word, lets its copies land and returns —
+ * without any fault. A negative value restores the full bound. Read by the
+ * kernels when they run (captured graphs included); set it only between
+ * steps. Synchronous. */
 CB_API int cb_debug_spin_limit(int32_t polls);
 
 /* ---- matrix products --------------------------------------------------------
