@@ -13,8 +13,10 @@
 // power of two that brings its largest magnitude into [2^14, 2^15), so
 // neither term leaves f16's range; a row's scale is applied to the finished
 // score, once a key. Weights take the value's scale: w_j = p_j·scale_j,
-// scaled by the power of two that brings the largest scale the row has seen
-// to 2^14 (it rises like the running maximum, and the sums with it).
+// scaled by the power of two that brings the largest of them that the row has
+// seen to 2^14 (it is kept like the running maximum, and the sums with it). It
+// is not the largest scale's: a key of large values and no weight would leave
+// the others few bits, or none.
 //
 // A masked key's weight is a chosen zero, never 0 times something, and its
 // score a chosen −∞: what it holds does not reach the row. In an 8-bit cache
@@ -60,6 +62,7 @@ namespace cb {
 namespace {
 
 constexpr uint32_t kKeys = 16;   // keys a tile
+constexpr float kLeastUnit = 0x1p-111f;   // 2^14 over it is a normal number
 constexpr uint32_t kAll = kAllLanes;
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
 
     float o[MT][D / 8][4];
     float top[MT][2], sum[MT][2];
-    float unit[MT][2];   // Q8: the power of two a row's value scales are held against
+    float unit[MT][2];   // Q8: the power of two a row's p·scale are held against
     const uint32_t mine = tile0 + warp < tile1 ? (tile1 - tile0 - warp + W - 1u) / W : 0u;
 
     auto pass = [&](const bool scalar) {
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
 #pragma unroll
             for (uint32_t n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.0f;
             top[m][0] = top[m][1] = kNegInf;
-            unit[m][0] = unit[m][1] = 0x1p-111f;   // 2^14 over it is a normal number
+            unit[m][0] = unit[m][1] = kLeastUnit;
             sum[m][0] = sum[m][1] = 0.0f;
         }
         for (uint32_t it = 0; it < mine; ++it) {
@@ -361,6 +364,9 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
             for (uint32_t m = 0; m < MT; ++m) {
                 float p[2][4];
                 uint32_t hidden = 0;
+                // p is at most 1, so no p·scale can pass a unit that no scale passes
+                // (the weights have room for twice it): seen before the scores are
+                const bool wide = F::Q8 && __any_sync(kAll, most > 2.0f * fminf(unit[m][0], unit[m][1]));
 #pragma unroll
                 for (uint32_t n = 0; n < 2; ++n)
 #pragma unroll
@@ -389,36 +395,7 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
                     top[m][k] = now;
                     alpha[m][k] = now == kNegInf ? 1.0f : ex2(was - now);
                 }
-                float lift[2] = {1.0f, 1.0f};   // what a new unit makes of the sums so far
-                bool moved = false;
-                if (F::Q8) {
-                    float big[2] = {most, most};
-                    if (!plain) {   // the scales of the row's visible keys alone
-                        big[0] = big[1] = 0.0f;
-#pragma unroll
-                        for (uint32_t n = 0; n < 2; ++n)
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i)
-                                if (!(hidden >> (4u * n + i) & 1u)) big[i >> 1] = fmaxf(big[i >> 1], vs[n][i & 1u]);
-                    }
-                    const float inf = __builtin_huge_valf();
-                    moved = __any_sync(kAll, (big[0] > unit[m][0] && big[0] < inf) || (big[1] > unit[m][1] && big[1] < inf));
-                    if (moved) {
-#pragma unroll
-                        for (uint32_t k = 0; k < 2; ++k) {
-                            float b = big[k] < inf ? big[k] : 0.0f;
-                            b = fmaxf(b, __shfl_xor_sync(kAll, b, 1));
-                            b = fmaxf(b, __shfl_xor_sync(kAll, b, 2));
-                            // the power of two at or above it, kept where 2^14 over it is a normal number
-                            const float up = fmaxf(unit[m][k], __uint_as_float(min((__float_as_uint(b) + 0x007FFFFFu) >> 23, 253u) << 23));
-                            lift[k] = unit[m][k] / up;
-                            unit[m][k] = up;
-                        }
-                    }
-                }
-                // 2^14 over the units, by their exponents
-                const float down[2] = {F::Q8 ? __uint_as_float((268u - (__float_as_uint(unit[m][0]) >> 23)) << 23) : 16384.0f,
-                                       F::Q8 ? __uint_as_float((268u - (__float_as_uint(unit[m][1]) >> 23)) << 23) : 16384.0f};
+                // p, added to its row's sum, then p·scale
                 const float base[2] = {top[m][0] == kNegInf ? 0.0f : top[m][0], top[m][1] == kNegInf ? 0.0f : top[m][1]};
                 float add[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -428,7 +405,7 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
                         const uint32_t k = i >> 1, x = i & 1u;
                         const float w = ex2(p[n][i] - base[k]);
                         add[k] += w;
-                        p[n][i] = w * (vs[n][x] * down[k]);
+                        p[n][i] = F::Q8 ? w * vs[n][x] : w;
                     }
                 if (!plain) {   // a hidden key's scale may be anything
 #pragma unroll
@@ -437,20 +414,54 @@ __global__ void __launch_bounds__(F::W * 32, F::kResident) tree_attention_kernel
                         for (uint32_t i = 0; i < 4; ++i)
                             if (hidden >> (4u * n + i) & 1u) p[n][i] = 0.0f;
                 }
+                // The unit falls with the sums when the maximum rises, and is
+                // raised where some p·scale passes it; what both make of the
+                // outputs so far:
+                float keep[2] = {alpha[m][0], alpha[m][1]};
+                bool moved = __any_sync(kAll, risen);
+                if (F::Q8 && (moved || wide)) {
+                    float big[2];
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        big[k] = fmaxf(fmaxf(p[0][2 * k], p[0][2 * k + 1]), fmaxf(p[1][2 * k], p[1][2 * k + 1]));
+                        if (!(big[k] < __builtin_huge_valf())) big[k] = 0.0f;
+                    }
+                    moved = moved || __any_sync(kAll, big[0] > 2.0f * unit[m][0] || big[1] > 2.0f * unit[m][1]);
+                    if (moved) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            float b = fmaxf(big[k], __shfl_xor_sync(kAll, big[k], 1));
+                            b = fmaxf(b, __shfl_xor_sync(kAll, b, 2));
+                            b = fmaxf(fmaxf(b, unit[m][k] * alpha[m][k]), kLeastUnit);
+                            // the power of two at or above it, kept where 2^14 over it is a normal number
+                            const uint32_t now = min((__float_as_uint(b) + 0x007FFFFFu) >> 23, 253u);   // its exponent
+                            // unit over now, at most 1 / alpha where alpha is not 0
+                            const int over = static_cast<int>((__float_as_uint(unit[m][k]) >> 23) - now) + 127;
+                            keep[k] *= __uint_as_float(static_cast<uint32_t>(min(max(over, 0), 254)) << 23);
+                            unit[m][k] = __uint_as_float(now << 23);
+                        }
+                    }
+                }
+                // 2^14 over the units, by their exponents
+                const float down[2] = {F::Q8 ? __uint_as_float((268u - (__float_as_uint(unit[m][0]) >> 23)) << 23) : 16384.0f,
+                                       F::Q8 ? __uint_as_float((268u - (__float_as_uint(unit[m][1]) >> 23)) << 23) : 16384.0f};
+#pragma unroll
+                for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) p[n][i] *= down[i >> 1];
                 sum[m][0] = fmaf(sum[m][0], alpha[m][0], add[0]);
                 sum[m][1] = fmaf(sum[m][1], alpha[m][1], add[1]);
                 split2(p[0][0], p[0][1], phi[m].x, plo[m].x);
                 split2(p[0][2], p[0][3], phi[m].y, plo[m].y);
                 split2(p[1][0], p[1][1], phi[m].z, plo[m].z);
                 split2(p[1][2], p[1][3], phi[m].w, plo[m].w);
-                if (__any_sync(kAll, risen) || moved) {
-                    const float f0 = alpha[m][0] * lift[0], f1 = alpha[m][1] * lift[1];
+                if (moved) {
 #pragma unroll
                     for (uint32_t n = 0; n < D / 8; ++n) {
-                        o[m][n][0] *= f0;
-                        o[m][n][1] *= f0;
-                        o[m][n][2] *= f1;
-                        o[m][n][3] *= f1;
+                        o[m][n][0] *= keep[0];
+                        o[m][n][1] *= keep[0];
+                        o[m][n][2] *= keep[1];
+                        o[m][n][3] *= keep[1];
                     }
                 }
                 if (!F::Q8 && scalar) {

@@ -12,8 +12,10 @@
 //
 // A key being a lane, its scale is a number of the thread that holds it, and
 // a row's maximum runs across lanes. It is not found for every tile: the
-// weights are taken against a base that only has to keep them in f16's
-// range, and it is raised (with the sums) when some score passes it by 2^8.
+// weights are taken against a base, and their products with the scales
+// against a unit, that only have to keep them in f16's range, and both are
+// raised (with the sums) when some p passes the base, or some p·scale the
+// unit, by 2^8.
 // Otherwise a tile costs one barrier-with-or of the eight warps of each half
 // of the rows.
 //
@@ -84,7 +86,8 @@ constexpr uint32_t kMostSequences = 1024;
 constexpr uint32_t kScaleTiles = 8;             // tiles whose scales are held: copies run at most six ahead of the softmax
 constexpr uint32_t kPolls = 1u << 20;           // of a wait: a large fraction of a second at least
 constexpr float kRise = 8.0f;                   // log2 units a weight may pass its base by
-constexpr float kWeightTop = 128.0f;            // 2^15 / 2^kRise: a largest-scale weight at its base
+constexpr float kWeightTop = 128.0f;            // 2^15 / 2^kRise: a weight whose p·scale is its row's unit
+constexpr float kLeastUnit = -100.0f;           // log2
 
 template <uint32_t D_, bool Q8_, uint32_t RT_>
 struct Form {
@@ -142,14 +145,14 @@ struct Info {
     bool even_factor, even_weight[2];   // every row's (of a half) is the same
     uint64_t mask[64];
     uint32_t first[64];
-    float unit[64];            // the power of two the row's value scales are held against
+    float unit[64];            // log2 of the power of two the row's p·scale are held against
     __align__(8) float shift[64], sums[64];   // what a raised base adds to scores, makes of sums
     float outs[64];                           // and of outputs
     int found[4][64];          // a quadrant's largest score, ordered as an integer
-    uint32_t scale[4][64];     // and its largest visible value scale (bits)
+    int weighty[4][64];        // and its largest log2 of p·scale, likewise
     float total[4][64];
     uint32_t unset[2];         // a half's live rows that have seen no key yet
-    float least_unit[2];       // of the rows that have
+    float least_unit[2];       // of the rows that have (log2)
     uint32_t latest, context;  // tiles from one to before the other are seen whole by every row
     uint32_t last, abort, polls, tmem;
     uint32_t first_cta, last_cta;   // of a divided pair
@@ -289,7 +292,15 @@ __device__ __noinline__ uint64_t sight_of(const Info& info, uint32_t e) {
     return sight;
 }
 
-// One warp of a half: from the tile's largest scores and scales, each row's
+// 2^x of a whole number up to 127; 0 below −126.
+__device__ __forceinline__ float exp2i(float x) { return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(x), -127) + 127) << 23); }
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One warp of a half: from the tile's largest scores and p·scale, each row's
 // new base and unit, and what they make of what it has (info.shift, sums,
 // outs). A lane a row.
 template <class F>
@@ -297,12 +308,11 @@ __device__ __forceinline__ void raise_bases(Info& info, uint32_t half, uint32_t 
     constexpr uint32_t kRows = F::RT / 2;
     const uint32_t r = half * kRows + lane % kRows;
     const bool mine = lane < kRows;
-    int v = info.found[0][r];
-    uint32_t w = info.scale[0][r];
+    int v = info.found[0][r], w = F::Q8 ? info.weighty[0][r] : 0;
 #pragma unroll
     for (int k = 1; k < 4; ++k) {
         v = max(v, info.found[k][r]);
-        w = max(w, info.scale[k][r]);
+        if (F::Q8) w = max(w, info.weighty[k][r]);
     }
     const float top = unordered(v);   // relative to the base; ordered(NaN) is below −∞'s
     const bool unset = info.unset[half] >> (lane % kRows) & 1u;
@@ -311,52 +321,58 @@ __device__ __forceinline__ void raise_bases(Info& info, uint32_t half, uint32_t 
         shift = top;
         if (!unset) keep = ex2(-top);
     }
-    const float was = info.unit[r];
-    float now = F::Q8 ? fmaxf(was, __uint_as_float(min((w + 0x007FFFFFu) >> 23, 253u) << 23)) : 1.0f;
     const bool set = mine && info.weight[r] != 0.0f && (!unset || top > kNegInf);
-    // one unit for all rows where theirs are within 2^6 of each other
-    const uint32_t least = __reduce_min_sync(kAllLanes, set ? __float_as_uint(now) : 0x7F800000u);
-    const uint32_t most = __reduce_max_sync(kAllLanes, set ? __float_as_uint(now) : 0u);
-    const bool even = most == 0u || (most >> 23) - (least >> 23) <= 6u;
-    if (F::Q8 && even && most != 0u) now = __uint_as_float(most);
+    const float was = info.unit[r];
+    float now = 0.0f;
+    bool even = true;
+    if (F::Q8) {
+        // The unit falls with the sums when the base rises, and is raised to the tile's largest p·scale.
+        const float heaviest = unordered(w) - shift;
+        now = unset ? kLeastUnit : fmaxf(ceilf(was - shift), kLeastUnit);
+        if (heaviest > now) now = fminf(ceilf(heaviest), 126.0f);   // kWeightTop over it stays a normal number
+        // one unit for all rows where theirs are within 2^6 of each other
+        const int most = __reduce_max_sync(kAllLanes, set ? static_cast<int>(now) : -1000);
+        const int least = __reduce_min_sync(kAllLanes, set ? static_cast<int>(now) : 1000);
+        even = most - least <= 6;   // or no row is set
+        if (even && most > -1000) now = static_cast<float>(most);
+        if (lane == 0) info.least_unit[half] = static_cast<float>(most == -1000 ? static_cast<int>(kLeastUnit) : even ? most : least);
+    }
     const uint32_t now_set = __ballot_sync(kAllLanes, set);
     if (mine) {
         info.shift[r] = -shift;
         info.sums[r] = keep;
         info.base[r] -= shift;
-        info.outs[r] = F::Q8 ? keep * (was / now) : keep;
+        // nothing was summed of an unset row; else now >= was − shift, so that this is at most 1
+        info.outs[r] = F::Q8 ? (unset || keep == 0.0f ? keep : keep * exp2i(was - now)) : keep;
         info.unit[r] = now;
-        if (F::Q8 && info.weight[r] != 0.0f) info.weight[r] = kWeightTop / now;
+        if (F::Q8 && info.weight[r] != 0.0f) info.weight[r] = kWeightTop * exp2i(-now);
     }
     __syncwarp();
     if (lane == 0) {
         info.unset[half] &= ~now_set;
-        info.least_unit[half] = __uint_as_float(even ? most : least);
         info.even_weight[half] = even;
     }
 }
 
 // New bases for the rows of a half, by all its warps: each row's largest score
-// and value scale of the tile, then scores, sums and the outputs so far moved
+// and p·scale of the tile, then scores, sums and the outputs so far moved
 // to the new bases and units. `it`: the tile's number, `after` whether the
 // stretch has products before it. In line and without a call, so that what
 // the loop holds stays in registers.
 template <class F>
-__device__ __forceinline__ void raise_all(Info& info, float (&e)[F::RH], float (&sum)[F::RH], float scale, bool plain, uint32_t mine,
-                                          uint32_t it, bool after, bool folded, uint32_t lanes) {
+__device__ __forceinline__ void raise_all(Info& info, float (&e)[F::RH], float (&sum)[F::RH], float scale, uint32_t it,
+                                          bool after, bool folded, uint32_t lanes) {
     constexpr uint32_t D = F::D, RT = F::RT, RH = F::RH;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, group = warp >> 2, quad = warp & 3u, half = group / kColumnParts;
     const uint32_t r0 = group * RH;
-    const bool counts = scale < __builtin_huge_valf() && scale > 0.0f;
-    uint32_t w = 0;
-    if (F::Q8 && plain) w = __reduce_max_sync(kAllLanes, counts ? __float_as_uint(scale) : 0u);
+    const float log_scale = F::Q8 && scale > 0.0f && scale < __builtin_huge_valf() ? lg2(scale) : kNegInf;
 #pragma unroll
     for (uint32_t i = 0; i < RH; ++i) {
         const int v = __reduce_max_sync(kAllLanes, ordered(e[i]));
-        if (F::Q8 && !plain) w = __reduce_max_sync(kAllLanes, (mine >> i & 1u) && counts ? __float_as_uint(scale) : 0u);
-        if (lane == 0) {
-            info.found[quad][r0 + i] = v;
-            info.scale[quad][r0 + i] = w;
+        if (lane == 0) info.found[quad][r0 + i] = v;
+        if (F::Q8) {
+            const int w = __reduce_max_sync(kAllLanes, ordered(e[i] + log_scale));
+            if (lane == 0) info.weighty[quad][r0 + i] = w;
         }
     }
     half_sync(half);
@@ -532,16 +548,19 @@ __device__ __noinline__ void soften(Info& info, char* smem, uint32_t tmem) {
         float most[2] = {kNegInf, kNegInf};
 #pragma unroll
         for (uint32_t j = 0; j < RH; j += 2) most[j / 2 % 2] = max3(most[j / 2 % 2], e[j], e[j + 1]);
-        bool raise = fmaxf(most[0], most[1]) > kRise;
+        // p may pass its base, and p·scale its row's unit, by 2^kRise
+        float past = 0.0f;   // log2 of the scale over the least unit
+        if (F::Q8 && scale.y < __builtin_huge_valf()) past = fmaxf(lg2(scale.y) - info.least_unit[half], 0.0f);
+        bool raise = fmaxf(most[0], most[1]) + past > kRise;
         raise |= (info.unset[half] & half_sight) != 0;
-        if (F::Q8) raise |= half_sight != 0 && scale.y > info.least_unit[half] && scale.y < __builtin_huge_valf();
-        if (half_any(half, raise)) raise_all<F>(info, e, sum, scale.y, plain, mine, it, t > 0, t >= kFold, lanes);   // rare
+        if (half_any(half, raise)) raise_all<F>(info, e, sum, scale.y, it, t > 0, t >= kFold, lanes);   // rare
         const uint32_t pb = it % F::kWeights;
         wait(&info.pempty[pb], (it / F::kWeights & 1u) ^ 1u, info);
         char* to = smem + F::kPAt + pb * F::kP;
         // p = 2^e, added to its row's sum; its weight p·scale·factor in two terms.
-        const bool simple = plain && info.even_weight[half];   // every key seen, one weight factor
         const float down = scale.y * info.weight[half * (RT / 2)];
+        // every key seen, one weight factor, and one that does not pass f32's range where p·scale does not
+        const bool simple = plain && info.even_weight[half] && (!F::Q8 || down < __builtin_huge_valf());
 #pragma unroll
         for (uint32_t i = 0; i < RH; i += 8) {
             uint32_t hi[4], lo[4];
@@ -554,7 +573,7 @@ __device__ __noinline__ void soften(Info& info, char* smem, uint32_t tmem) {
                     sum[i + j + k] += p;
                     w[k] = p * down;
                     if (!simple) {
-                        w[k] = p * (scale.y * info.weight[r0 + i + j + k]);
+                        w[k] = p * scale.y * info.weight[r0 + i + j + k];
                         if (!(mine >> (i + j + k) & 1u)) w[k] = 0.0f;   // a hidden key's scale may be anything
                     }
                 }
@@ -986,7 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_tensor_kernel(cons
             if (live) row_sight(a, step, s, node, mask, first);
             info.mask[r] = mask;
             info.first[r] = first;
-            info.unit[r] = 0x1p-100f;
+            info.unit[r] = kLeastUnit;
             info.base[r] = 0.0f;
             info.weight[r] = live ? (F::Q8 ? kWeightTop * 0x1p100f : kWeightTop) : 0.0f;
         }
@@ -1067,7 +1086,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_tensor_kernel(cons
                 const uint32_t unset = __ballot_sync(kAllLanes, live);
                 if (lane == 0) {
                     info.unset[half] = unset;
-                    info.least_unit[half] = 0x1p-100f;
+                    info.least_unit[half] = kLeastUnit;
                 }
             }
             late = __reduce_max_sync(kAllLanes, late);
