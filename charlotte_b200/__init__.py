@@ -348,20 +348,28 @@ class Plan:
     """A kernel entry point with its arguments filled in once, for a program
     that makes the same call every step: calling it enqueues the launch on
     `stream` (default: torch's current stream). It holds the tensors it was
-    given, and a tree attention's workspace unless one was."""
+    given, and a tree attention's workspace unless one was; that one is ready
+    for a call on any stream, and calls that overlap on the GPU need a plan
+    each."""
 
     _structs = {"cache_write": CacheWrite, "cache_read": CacheRead, "tree_attention": TreeAttention,
                 "verify": Verify, "cache_keep": CacheKeep}
 
     def __init__(self, entry: str, fields: dict):
         self._keep = []
+        self._streams = None   # those that a workspace of the plan's own is known on
         self.args = self._fill(self._structs[entry](), fields)
         if entry == "tree_attention" and fields.get("workspace") is None:
             import torch
             need = lib().cb_tree_attention_bytes(ctypes.byref(self.args))
             if need == 0:
                 raise CharlotteError(ERROR_INVALID, last_error())
-            self.use_workspace(torch.zeros(need, dtype=torch.uint8, device=fields["out"].device))
+            device = fields["out"].device
+            self.use_workspace(torch.zeros(need, dtype=torch.uint8, device=device))
+            home = torch.cuda.current_stream(device)
+            if not torch.cuda.is_current_stream_capturing():
+                home.synchronize()   # zeroed before a call on any stream
+            self._streams = {home.cuda_stream}
         self._ref = ctypes.byref(self.args)
         self._fn = getattr(lib(), f"cb_{entry}_run")
 
@@ -379,11 +387,20 @@ class Plan:
     def use_workspace(self, workspace) -> None:
         """A tree attention's workspace from here on (a zeroed uint8 cuda tensor, which several plans may share whose
         calls follow one another)."""
-        self.workspace = workspace
+        self.workspace, self._streams = workspace, None
         self.args.workspace, self.args.workspace_bytes = workspace.data_ptr(), workspace.numel()
 
+    def _used_on(self, handle: int) -> None:
+        """The plan's own workspace is not handed out again, once the plan is gone, before that stream's work is done."""
+        import torch
+        self.workspace.record_stream(torch.cuda.ExternalStream(handle, device=self.workspace.device))
+        self._streams.add(handle)
+
     def __call__(self, stream=None, flags: int = 0) -> None:
-        status = self._fn(self._ref, flags, _stream(stream))
+        handle = _stream(stream)
+        if self._streams is not None and handle not in self._streams:
+            self._used_on(handle)
+        status = self._fn(self._ref, flags, handle)
         if status != OK:
             check(status)
 
