@@ -12,6 +12,25 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (a B200); runs the CUDA kernels")
 
 
+# Suites that run code compiled from the reference's own sources.
+REFERENCE_SIDE = {
+    "test_program_gpu": ("integration", "libcharlotte_program.so"),
+    "test_encoder_program_gpu": ("integration", "libcharlotte_program.so"),
+    "test_oracle_pins_gpu": ("oracle", "_ref", "libcharlotte_ref.so"),
+}
+
+
+def pytest_collection_modifyitems(items):
+    """Skips the suites whose reference-side library was not built because
+    there were no sources to build it from. Where there are, they run, and a
+    missing library fails them."""
+    import oracle
+    for item in items:
+        library = REFERENCE_SIDE.get(item.module.__name__)
+        if library and not os.path.exists(os.path.join(ROOT, *library)) and oracle.reference_root() is None:
+            item.add_marker(pytest.mark.skip(reason="the reference sources were absent when its side would have been built"))
+
+
 @pytest.fixture(scope="session")
 def cuda():
     """The CUDA device for GPU tests. A GPU test never skips: without a device
