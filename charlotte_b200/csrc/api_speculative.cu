@@ -108,6 +108,7 @@ int cb_cache_write_run(const cb_cache_write* w, uint32_t flags, void* stream) {
     if (!aligned16(w->query) || !aligned16(w->query_out) || !aligned16(w->key) || !aligned16(w->value) ||
         !aligned16(w->query_gain) || !aligned16(w->key_gain))
         return fail(CB_ERROR_INVALID, "%s: rows and gains must be 16-byte aligned", who);
+    if (!aligned4(w->turns) || !aligned4(w->factors)) return fail(CB_ERROR_INVALID, "%s: unaligned turns or factors", who);
     if (w->tokens == 0 || w->sequences == 0) return CB_OK;
     return launched(cache_write_run(*w, static_cast<cudaStream_t>(stream), flags & CB_RUN_PDL), who);
 }
@@ -152,6 +153,8 @@ int cb_verify_run(const cb_verify* v, uint32_t flags, void* stream) {
     if (int rc = step_arguments(v->nodes, v->nodes, v->ancestors, 0, v->tokens, true, who)) return rc;
     if (!aligned16(v->candidates) || !aligned16(v->draft_candidates))
         return fail(CB_ERROR_INVALID, "%s: candidate lists must be 16-byte aligned", who);
+    if (!aligned4(v->ids) || !aligned4(v->uniforms) || !aligned4(v->path) || !aligned4(v->kept) || !aligned4(v->sampled))
+        return fail(CB_ERROR_INVALID, "%s: unaligned ids, uniforms or outputs", who);
     if (int rc = sampling_arguments(v->target, "target")) return rc;
     if (v->draft_candidates)
         if (int rc = sampling_arguments(v->draft, "draft")) return rc;
@@ -166,6 +169,7 @@ int cb_cache_keep_run(const cb_cache_keep* k, uint32_t flags, void* stream) {
     if (int rc = step_arguments(k->lengths, k->kept, nullptr, k->position0, k->tokens, true, who)) return rc;
     if (k->tokens > k->cache.slots)
         return fail(CB_ERROR_INVALID, "%s: %u rows in %u slots", who, k->tokens, k->cache.slots);
+    if (!aligned4(k->path) || !aligned4(k->new_lengths)) return fail(CB_ERROR_INVALID, "%s: unaligned path or new lengths", who);
     if (k->new_lengths && k->new_lengths == k->lengths)
         return fail(CB_ERROR_INVALID, "%s: lengths updated in place", who);
     if (k->layers > 65535) return fail(CB_ERROR_INVALID, "%s: %u layers", who, k->layers);
