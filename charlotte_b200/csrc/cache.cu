@@ -13,6 +13,7 @@
 
 #include <cstdint>
 
+#include "api_common.h"
 #include "cache.cuh"
 #include "kernels.h"
 #include "numerics.cuh"
@@ -310,7 +311,9 @@ cudaError_t cache_write_run(const cb_cache_write& a, cudaStream_t stream, bool p
     const uint32_t lanes = (a.query_heads + 2u * a.cache.kv_heads) * (a.cache.head_dim / 8u);
     const uint32_t threads = lanes < 512u ? (lanes + 31u) / 32u * 32u : 512u;
     const size_t smem = a.cache.head_dim * sizeof(float);
-    if (static_cast<uint64_t>(a.tokens) * a.sequences <= 148u * (2048u / threads))
+    const int sms = sm_count();
+    if (sms <= 0) return cudaErrorNoDevice;
+    if (static_cast<uint64_t>(a.tokens) * a.sequences <= static_cast<uint32_t>(sms) * (2048u / threads))
         return launch(cache_write_kernel<1>, dim3(a.tokens, a.sequences), threads, smem, stream, pdl, a);
     return launch(cache_write_kernel<2>, dim3((a.tokens - 1u) / 2u + 1u, a.sequences), threads, 2u * smem, stream, pdl, a);
 }
