@@ -45,6 +45,17 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Two sums, whose steps go beside one another.
+__device__ __forceinline__ float2 warp_sums(float a, float b) {
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+        const float x = __shfl_xor_sync(kAll, a, k), y = __shfl_xor_sync(kAll, b, k);
+        a += x;
+        b += y;
+    }
+    return make_float2(a, b);
+}
+
 // Sum of the values before this lane's pair (a, b), in list order.
 __device__ __forceinline__ float sum_before(float a, float b, uint32_t lane) {
     float run = a + b;
@@ -242,24 +253,34 @@ __global__ void __launch_bounds__(64) verify_kernel(const VerifyArgs args) {
                         }
                     }
                 }
-                rest[0] = fmaxf(r.p[0] - on_target[0] / mass, 0.0f);   // a subnormal mass has no finite inverse
-                rest[1] = fmaxf(r.p[1] - on_target[1] / mass, 0.0f);
+                const float scale = 1.0f / mass;
+                float given[2] = {on_target[0] * scale, on_target[1] * scale};
+                if (!(scale < __builtin_huge_valf())) {   // a subnormal mass
+                    given[0] = on_target[0] / mass;
+                    given[1] = on_target[1] / mass;
+                }
+                rest[0] = fmaxf(r.p[0] - given[0], 0.0f);
+                rest[1] = fmaxf(r.p[1] - given[1], 0.0f);
             } else {
                 rest[0] = r.token[0] == t ? 0.0f : r.p[0];
                 rest[1] = r.token[1] == t ? 0.0f : r.p[1];
             }
+            float total;
             if (have) {
                 // What is left of q, summed and not one less what is gone: a draft
                 // sure of its first token leaves its siblings 1e-8 and less, which
                 // that difference rounds away. Nothing left: every later sibling's
                 // probability is 0, and it is refused.
                 forget(q, t);
-                mass = warp_sum(q.p[0] + q.p[1]);
+                const float2 both = warp_sums(rest[0] + rest[1], q.p[0] + q.p[1]);
+                total = both.x;
+                mass = both.y;
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
                     if (r.token[c] == t) on_target[c] = 0.0f;
+            } else {
+                total = warp_sum(rest[0] + rest[1]);
             }
-            const float total = warp_sum(rest[0] + rest[1]);
             if (total > 0.0f) {
                 const float scale = 1.0f / total;
                 r.p[0] = rest[0] * scale;
