@@ -15,7 +15,7 @@ import math
 
 import numpy as np
 
-from . import CACHE_Q8, GATED, QKV, CharlotteError, check, lib, matmul, plan, rope_turns, run
+from . import CACHE_Q8, ERROR_STEP, GATED, QKV, CharlotteError, check, lib, matmul, plan, rope_turns, run
 from . import model as M
 from . import synth
 
@@ -189,7 +189,8 @@ class SpeculativeDecoder:
         in DRAW (greedy); `uniforms` [sequences, nodes], which a target with a temperature needs; `draft`: the drafting model's
         candidates [sequences, nodes, 64, 2] (int32, cuda), None where each drafted token was certain. Returns each
         sequence's new tokens, the last of them the next tree's row 0. A tree with a row past the context is a ValueError,
-        and nothing runs; a kernel whose wait ran out is a CharlotteError, and the step can be taken again."""
+        and nothing runs; a kernel whose wait ran out and logits that are not finite are a CharlotteError, and the step
+        can be taken again."""
         target = DRAW | (sampling or {})
         if target["temperature"] > 0 and uniforms is None:
             raise ValueError("a target with a temperature draws by uniform numbers, and none are given")
@@ -209,6 +210,8 @@ class SpeculativeDecoder:
             keep()
         path, kept, sampled = (x.cpu().numpy() for x in (self.path, self.kept, self.sampled))
         self._check_waits()   # before the lengths, so that a failed step's rows are no entries
+        if sampled[:, 1].any():
+            raise CharlotteError(ERROR_STEP, f"sequences {np.flatnonzero(sampled[:, 1]).tolist()}: the first candidate of a kept row is not finite")
         self.lengths.copy_(self.new_lengths)
         return [[int(trees[s][0][i]) for i in path[s, 1:kept[s]]] + [int(sampled[s, 0])] if kept[s] else []
                 for s in range(self.sequences)]

@@ -50,3 +50,19 @@ def test_a_failed_prompt_is_an_error_and_commits_nothing(cuda, short_waits):
     short_waits(-1)
     assert d.lengths.tolist() == [2]
     cb.check(cb.lib().cb_fault_check(None))
+
+
+def test_logits_that_are_not_finite_are_an_error(cuda):
+    """As the exact decoder's record says of its draw; the step is not committed, and others go on."""
+    m = M.synthesize(M.tiny("qwen3"), seed=3)
+    d = S.SpeculativeDecoder(m, 2, 3)
+    d.prefill([[5, 6, 7], [8, 9]])
+    step = [([7, 1], [-1, 0]), ([9], [-1])]
+    gain = d.output_norm.clone()
+    d.output_norm.fill_(float("nan"))
+    with pytest.raises(cb.CharlotteError, match="not finite") as e:
+        d.step(step)
+    assert e.value.status == cb.ERROR_STEP
+    assert d.lengths.tolist() == [2, 1]
+    d.output_norm.copy_(gain)
+    assert all(d.step(step))
