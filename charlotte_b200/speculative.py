@@ -145,6 +145,12 @@ class SpeculativeDecoder:
             if n and length + n > self.arch.context:
                 raise ValueError(f"sequence {s}: positions past the context of {self.arch.context} ({length} + {n})")
 
+    def _in_vocabulary(self, tokens) -> None:
+        """Tokens a sequence holds: a drafted one that is not the model's is refused by verification instead."""
+        for t in tokens:
+            if not 0 <= t < self.arch.vocab:
+                raise ValueError(f"token {t} of a vocabulary of {self.arch.vocab}")
+
     def _set(self, trees) -> None:
         """trees: for each sequence its rows' (tokens, ancestor masks); no rows: it takes no part."""
         ids = np.zeros((self.sequences, self.nodes), np.uint32)
@@ -165,8 +171,9 @@ class SpeculativeDecoder:
 
     def prefill(self, prompts) -> None:
         """Writes each sequence's prompt but its last token, which the first step takes as its row 0. A prompt that does
-        not fit its sequence's context is a ValueError, and nothing runs."""
+        not fit its sequence's context, and a token that is not the model's, is a ValueError, and nothing runs."""
         self._within_context(self.lengths.tolist(), [len(p) - 1 for p in prompts])
+        self._in_vocabulary(t for p in prompts for t in p)
         done, start = [0] * self.sequences, self.lengths.clone()
         while any(d < len(p) - 1 for d, p in zip(done, prompts)):
             trees = []
@@ -196,6 +203,7 @@ class SpeculativeDecoder:
             raise ValueError("a target with a temperature draws by uniform numbers, and none are given")
         masks = [(tokens, ancestors(parents)) for tokens, parents in trees]
         self._within_context(self.lengths.tolist(), [max((x.bit_count() for x in m), default=0) for _, m in masks])
+        self._in_vocabulary(tokens[0] for tokens, _ in masks if len(tokens))
         self._set(masks)
         self._forward(logits=True)
         a, rows = self.arch, self.ids.shape[0]
