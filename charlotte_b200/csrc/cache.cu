@@ -30,8 +30,9 @@ namespace {
 // i and i + d/8 as in rope_kernel. The rows' angles are found once into shared
 // memory while their queries, keys and values are on their way. Bound: latency
 // (load, angles, norm, store, one after the other) while the rows fill the GPU
-// less than once: eight trees of 16 rows, 16 + 2·8 heads of 128, 3.8 us. Past
-// that, HBM and L2: a 2,047-row prompt of 32 + 2·8 heads of 64, 44 MB, 10.4 us.
+// less than once: eight trees of 16 rows, 16 + 2·8 heads of 128, 3.8 to 4.2 us. Past
+// that, latency of two waves and L2, which holds that much: a 2,047-row prompt of
+// 32 + 2·8 heads of 64, 44 MB, 10.4 to 11.1 us (4.1 TB/s).
 // Two rows a CTA have their loads and angles together, which helps once the
 // rows are more than the CTAs that fit at a time (that prompt 12.2 us with one
 // row) and costs a row's arithmetic before (those trees 5.0 us with two).
@@ -150,9 +151,12 @@ __global__ void __launch_bounds__(512, 2) cache_write_kernel(const cb_cache_writ
 // that a warp's stores are whole lines whatever the formats: the same piece of
 // kReadUnroll entries, their loads together, with the entry's slot stepped and
 // not divided out: with the divisions a store, one 16-code unit a thread, the
-// figures below were 7.1 and 27.8 us. Bound: HBM and L2 (a 4,096-entry ring of
-// 8 heads of 128 codes to f16 6.4 us; 64 times 777 entries of a head of 256 to f32
-// 23.4 us, 128 MB: 5.5 TB/s).
+// figures below were 7.1 and 27.8 us. Bound: launch and one dependent load, then
+// L2 and HBM. Called again on the same cache, whose codes then wait in L2: a
+// 4,096-entry ring of 8 heads of 128 codes to f16 6.4 us, 64 times 777 entries of
+// a head of 256 to f32 23.4 us (128 MB read and written, 5.5 TB/s); on caches that
+// do not, 8.2 and 28.7 us. The same entries of an f16 cache, waiting in L2: to f16
+// 5.4 and 12.1 us, to f32 7.4 and 24.4.
 constexpr uint32_t kReadUnroll = 8;
 
 template <bool Q8, bool F32>
@@ -246,9 +250,9 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const cb_cache_read a, 
 // path[d] ≥ d), and no earlier move of the same column has written it. Eight
 // rows' loads go before their stores. Bound: for one layer latency (path, rows
 // and stores one after the other; eight sequences 3.2 us, 4.5 with keys and
-// values in one CTA); for a batch's layers HBM, reads and writes mixed in
-// pieces of a row (64 sequences of 28 layers, 117 MB, 28 us: 4.2 TB/s; 4 or 16
-// rows ahead take 28 and 29 us).
+// values in one CTA); for a batch's layers HBM (64 sequences of 28 layers, of 32
+// rows 11.7 moved, read and written 171 MB, 28.7 us: 6.0 TB/s; 4 or 16 rows ahead
+// take 28 and 29 us).
 __global__ void __launch_bounds__(256) cache_keep_kernel(const cb_cache_keep a) {
     __shared__ uint32_t path[kTreeRows];
     grid_dependency_wait();

@@ -36,10 +36,13 @@
 // the tree share the keys' fragments.
 //
 // Bound. A batch's decode is bound by instructions issued (two a cycle; the
-// copies, codes to f16 and two terms for every product): 64 sequences of one
-// row over 2k to 4k 8-bit keys 136 us (3.0 TB/s), 32 of 16 rows over 8k to 16k
-// 245 us (3.2 TB/s). A small step is latency: one row over 2,000 keys 9.8 us, 16 sequences
-// of 52 rows over a window of 512 (256 values) 17.5 us.
+// copies, codes to f16 and two terms for every product, of whose 16 rows a step
+// of 8 rows or fewer leaves half empty): 64 sequences of one row over 2k to 4k
+// keys of 128 values, 8-bit, 132 us (3.0 TB/s), of 64 values 95 us, of 256
+// values in one head 47 us (2.1 TB/s); f16 rows of 128, 16 sequences over 2,000,
+// 29 us (3.0 TB/s); 32 sequences of 16 rows over 8k to 16k 242 us (3.2 TB/s). A small step
+// is latency: one row over 2,000 keys 9.2 us, 16 sequences of 52 rows over a
+// window of 512 (256 values) 16.8 us.
 //
 // Fragments (mma.sync m16n8k16). The contraction order over d is free, so a
 // lane takes keys as 16-byte pieces of a row, four steps a piece; the columns

@@ -27,11 +27,16 @@
 // codes land in a ring and are made f16 by warps of their own.
 //
 // Bound. 32 trees of 32 nodes (64 rows a kv head of 128 values) over 8-bit
-// contexts of 16k to 32k keys: 665 to 715 us as the clocks go, that is 1.58
-// GB at 2.4 TB/s, and 377 GFLOP of both terms at 567 TFLOP/s, 2 us a tile. A tile moves 320 KB through shared memory, some 2,500 cycles at 128
-// bytes: 160 KB that the products read (64 rows are few for keys that are read
-// once a term), 32 KB of weights, 128 KB for codes to arrive and become f16.
-// With f16 rows of 64 values (8 trees of 96 rows over 4k to 8k keys, 84 to 89 us) a tile is the
+// contexts of 16k to 32k keys: 620 to 710 us as the clocks go, that is 1.58
+// GB at 2.2 to 2.5 TB/s and 377 GFLOP of both terms at 530 to 610 TFLOP/s, 2 us a
+// tile. Nothing is full: the issue slots half, the tensor pipe a quarter, and
+// shared memory, whose 320 KB a tile (160 that the products read, 64 rows being
+// few for keys that are read once a term, 32 of weights, 128 for codes to
+// arrive and become f16) are 2,500 cycles at 128 bytes, 1.3 us of the 2. The rest
+// is a chain that waits: with one stage of operands a tile's codes become f16
+// only once the products of the tile before are done with theirs, and the
+// softmax's warps all stand at one tile and its vote.
+// With f16 rows of 64 values (8 trees of 96 rows over 4k to 8k keys, 83 to 87 us) a tile is the
 // softmax's own chain, 1.5 us of waits, conversions and stores, and beginning
 // and ending a share takes 15 us.
 // Measured and not kept: the two terms side by side in S's columns (a sum more
@@ -68,16 +73,17 @@ namespace {
 constexpr uint32_t kTile = 128;                 // keys
 // Warps: of softmax (four to each group of rows), of loading (half of them
 // keys, half values, so that neither waits for the other's space), and one that
-// issues the products. Nothing of a role's loop may spill: the shared memory
-// taken leaves the L1 little, and a spilled word comes back from L2 (600
-// cycles).
+// issues the products. Little of a role's loop may spill: the shared memory
+// taken leaves the L1 little, and a spilled word may come back from L2 (600
+// cycles). 800 threads leave each 72 registers: the softmax keeps 4 to 28 bytes
+// in local memory, for 64 rows over f16 rows of 64 values 80, of 128 values 148.
 constexpr uint32_t kSoftWarps = 16, kLoadWarps = 8, kThreads = 32 * (kSoftWarps + kLoadWarps + 1);
 constexpr uint32_t kGroups = kSoftWarps / 4, kHalfThreads = kSoftWarps * 16, kColumnParts = kGroups / 2;
 constexpr uint32_t kPrefetch = 2;               // tiles brought to L2 ahead of the loads
 // Tiles whose products are summed in one accumulator. The tensor cores cut each
 // of a tile's eight sums short instead of rounding it, always towards zero: over
 // 300 tiles 4e-6 of the result. In runs of kFold tiles, added up in f32, it is
-// 5e-7 (in runs of 8 3e-7, of 24 7e-7, of 48 1.3e-6; three times that where few
+// 5e-7 (in runs of 8 3e-7, of 24 7e-7, of 48 1.3e-6; four times that where few
 // keys have most of the weight); a run's end takes 1.3 us.
 constexpr uint32_t kFold = 16;
 constexpr uint32_t kBegin = 6;                  // tiles' time that beginning a pair takes, for the shares

@@ -14,7 +14,7 @@
 // memory from the start, so no visited node waits for its own. The draft's
 // probabilities of the target's candidates (64 by 64 comparisons) are found
 // only where a child is refused. A chain of 6 greedy drafts 3.1 us; 256 trees of
-// 48 nodes with a draft's lists 19.8 us, the longest walk's ten nodes at 2 us
+// 48 nodes with a draft's lists 20.0 us, the longest walk's ten nodes at 2 us
 // each (34 us in the first form, one warp a sequence).
 #include <cuda_runtime.h>
 

@@ -590,7 +590,12 @@ CB_API const float* cb_decoder_device_logits(cb_decoder* d);
  * in slot e mod slots. NULL ancestors: a chain, each row after the one
  * before. NULL nodes: every row. NULL lengths: position0 for every sequence.
  * lengths, nodes and ancestors are read on the device, so a captured graph
- * follows them. lengths + tokens stay below 2^31. */
+ * follows them. lengths + tokens stay below 2^31.
+ * A row takes its entry's slot whether it is kept or not: what lay there is
+ * gone, and a later, smaller step that still reaches back to it would attend
+ * what the refused row left. Where steps draft, a ring therefore has window +
+ * tokens - 1 slots at least, and a cache without a window one for every
+ * entry and `tokens` more. */
 
 /* How a cache holds a head row of head_dim values. F16: as cb_rope writes
  * them. Q8: one byte a value, code = clamp(round_even(x · min(127/m,
@@ -669,15 +674,21 @@ CB_API int cb_cache_read_run(const cb_cache_read* r, uint32_t flags, void* strea
  * `window` positions before its own (0: all), and of the entries only those
  * whose slot no later one has taken. One row a sequence is a plain decode
  * step. A row that attends nothing, and a row past nodes[s], is zeros.
- * f32 queries enter the tensor cores in two f16 terms, so results differ
- * from f32 arithmetic by its rounding only. max_keys (host) bounds
+ * Queries and weights enter the tensor cores in two f16 terms, 22 of f32's 24
+ * bits, relative to a row's largest query and to its largest weight times
+ * value scale; results are mostly 2e-7 to 5e-7 of their norm off (f32
+ * arithmetic 3e-7 to 6e-7), 5e-6 at most in the tests. max_keys (host) bounds
  * lengths[s] + nodes[s] and sets how many parts a sequence's keys are
  * divided into; entries past it are not attended. `workspace`:
  * cb_tree_attention_bytes of device memory, 16-byte aligned, zeroed before
  * its first use (a run leaves it ready for the next, of these sizes or
  * others); runs that overlap on the GPU need one each. Large steps of many
- * rows a kv head run on the tcgen05 tensor cores, the others on mma.sync, with
- * the same accuracy; CB_RUN_TENSOR takes the first whatever the sizes. */
+ * rows a kv head run on the tcgen05 tensor cores, which cut sums short instead
+ * of rounding them (added up in f32 every 16 tiles of 128 keys: 2e-6 to 3e-6
+ * where few of 31,000 keys have most of the weight, 0.5e-6 to 1.9e-6 in the
+ * other form), the others on mma.sync; CB_RUN_TENSOR takes the first whatever
+ * the sizes. Its waits are bounded: one that ran out is in the fault word
+ * (cb_fault_check). */
 typedef struct cb_tree_attention {
     cb_cache cache;
     const float* query;          /* [sequences·tokens][query_heads][head_dim]           */
